@@ -3,13 +3,21 @@
 //
 //   p = softmax(teacher / T) over the row's entries, q = softmax(logits / T)
 //   loss = w T^2 sum_j p_j (log p_j - log q[id_j])
+//        = w T sum_j p_j (t_j - t* - (s[id_j] - s*) - T (ln S_t - ln S_s))
 //   dloss / dlogits_i = w T (q_i - sum of the p_j with id_j = i)
+//
+// where * is a row's largest logit and S its sum of exp((logit - *) / T).  The
+// second form is the one computed: the largest logit is subtracted first, so
+// that no term is as large as the logits are, whose common offset would cost
+// the loss its digits and whose finite masks (the type's lowest value) would
+// overflow when they are scaled.
 //
 // An entry whose id is outside [0, v) or whose logit is -inf is absent; a row
 // without entries has loss 0 and gradient 0.  One read of the logits and one
 // write of the gradient: a workgroup keeps its row in registers between the
 // maximum, the sum and the gradient.  Softmax statistics are float; the
 // gradient is rounded once, by its store.
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -76,17 +84,25 @@ __device__ inline float sum_block(float v, float* lds) {
 }
 
 // The teacher's side of a row in LDS: for each entry its id (-1: absent), its
-// logarithmic probability, and its probability.
+// logit less the row's largest, and its probability.
 struct Entries {
   int32_t* id;
-  float* logp;
+  float* below;
   float* p;
 };
 
-// Fills `e` and returns whether the row has an entry.
+// The factor of an exponent, finite for the smallest temperatures too (the
+// largest logit's exponent is 0 times it).
+__device__ inline float per_temperature(float c, float temperature) {
+  return fminf(c / temperature, FLT_MAX);
+}
+
+// Fills `e` and `log_sum`, the logarithm of the entries' sum of exponentials,
+// and returns whether the row has an entry.
 template <class Tr, int kThreads>
-__device__ inline bool load_entries(const DistillArgs& a, int64_t row, const Entries& e, float* lds) {
-  const float inv_t = 1.f / a.temperature;
+__device__ inline bool load_entries(const DistillArgs& a, int64_t row, const Entries& e, float* lds,
+                                    float& log_sum) {
+  const float inv_t = per_temperature(1.f, a.temperature);
   float top = -INFINITY;
   bool nan = false;
   for (int j = threadIdx.x; j < a.k; j += kThreads) {
@@ -95,45 +111,45 @@ __device__ inline bool load_entries(const DistillArgs& a, int64_t row, const Ent
                               : static_cast<const int32_t*>(a.ids)[at];
     float t = -INFINITY;
     if (i >= 0 && i < a.v)
-      t = (a.teacher_f32 ? static_cast<const float*>(a.teacher)[at]
-                         : Tr::ld(static_cast<const typename Tr::S*>(a.teacher)[at])) * inv_t;
+      t = a.teacher_f32 ? static_cast<const float*>(a.teacher)[at]
+                        : Tr::ld(static_cast<const typename Tr::S*>(a.teacher)[at]);
     e.id[j] = t != -INFINITY ? static_cast<int32_t>(i) : -1;
-    e.logp[j] = t;
+    e.below[j] = t;
     nan |= t != t;
     top = fmaxf(top, t);
   }
   top = max_block<kThreads>(nan ? INFINITY : top, lds);  // inf - inf is NaN again
   float sum = 0.f;
   for (int j = threadIdx.x; j < a.k; j += kThreads) {
-    const float p = e.id[j] >= 0 ? expf(e.logp[j] - top) : 0.f;
+    const float below = e.below[j] - top;
+    const float p = e.id[j] >= 0 ? expf(below * inv_t) : 0.f;
+    e.below[j] = below;
     e.p[j] = p;
     sum += p;
   }
   sum = sum_block<kThreads>(sum, lds);
-  const float log_sum = logf(sum);
-  for (int j = threadIdx.x; j < a.k; j += kThreads) {
-    e.p[j] /= sum;
-    e.logp[j] = e.logp[j] - top - log_sum;
-  }
+  log_sum = logf(sum);
+  for (int j = threadIdx.x; j < a.k; j += kThreads) e.p[j] /= sum;
   return top != -INFINITY;  // this thread's own entries are read next, or after a barrier
 }
 
-// Sum over the entries of p (log p - log q); x: the row's logits.
+// T times the sum over the entries of p (log p - log q); x: the row's logits,
+// top the largest of them, log_ratio the entries' logarithm less the logits'.
 template <class Tr, int kThreads>
 __device__ inline float divergence(const DistillArgs& a, const typename Tr::S* x, const Entries& e,
-                                   float lse, float* lds) {
-  const float inv_t = 1.f / a.temperature;
+                                   float top, float log_ratio, float* lds) {
+  const float shift = a.temperature * log_ratio;
   float term = 0.f;
   for (int j = threadIdx.x; j < a.k; j += kThreads)
     if (e.id[j] >= 0 && e.p[j] != 0.f)
-      term += e.p[j] * (e.logp[j] - (Tr::ld(x[e.id[j]]) * inv_t - lse));
+      term += e.p[j] * (e.below[j] - (Tr::ld(x[e.id[j]]) - top) - shift);
   return sum_block<kThreads>(term, lds);
 }
 
-// 2^(x c - top c) = exp((x - top) / T) with c = log2(e) / T.  A row whose
-// maximum is -inf gives NaN.
-__device__ inline float soft(float x, float c, float top_c) {
-  return __builtin_amdgcn_exp2f(fmaf(x, c, -top_c));
+// exp((x - top) / T) with c = log2(e) / T: exactly 1 for the largest.  A row
+// whose maximum is -inf gives NaN.
+__device__ inline float soft(float x, float c, float top) {
+  return __builtin_amdgcn_exp2f((x - top) * c);
 }
 
 // The gradient at the entries' places in [begin, end), over the q that the
@@ -204,7 +220,8 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
       for (int c = tid * kPack; c < whole; c += kThreads * kPack) f(c, load_words<S>(x + c));
     }
   };
-  const bool some = load_entries<Tr, kThreads>(a, row, e, lds);
+  float log_entries;
+  const bool some = load_entries<Tr, kThreads>(a, row, e, lds, log_entries);
   S* back = a.backprop ? static_cast<S*>(a.backprop) + row * a.v : nullptr;
   if (!some) {
     if (tid == 0) a.loss[row] = 0.f;
@@ -218,34 +235,33 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
     for (int j = 0; j < kPack; ++j) top = fmaxf(top, element<Tr>(w, j));
   });
   top = max_block<kThreads>(top, lds);
-  const float c2 = kLog2E / a.temperature, top_c = top * c2;
-  float sum = soft(rest, c2, top_c);
+  const float c2 = per_temperature(kLog2E, a.temperature);
+  float sum = soft(rest, c2, top);
   each([&](int, const Words<S>& w) {
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) sum += soft(element<Tr>(w, j), c2, top_c);
+    for (int j = 0; j < kPack; ++j) sum += soft(element<Tr>(w, j), c2, top);
   });
   sum = sum_block<kThreads>(sum, lds);
-  const float lse = top / a.temperature + logf(sum);
   const float weight = a.weights ? a.weights[row] : 1.f;
-  const float kl = divergence<Tr, kThreads>(a, x, e, lse, lds);
-  if (tid == 0) a.loss[row] = weight * a.temperature * a.temperature * kl;
+  const float kl = divergence<Tr, kThreads>(a, x, e, top, log_entries - logf(sum), lds);
+  if (tid == 0) a.loss[row] = weight * a.temperature * kl;
   if (!back) return;
 
   // The gradient may take the logits' own memory: what the entries need of
   // them is read before the first store.
   const float inv_sum = 1.f / sum, factor = weight * a.temperature;
   for (int j = tid; j < a.k; j += kThreads)
-    own[j] = e.id[j] >= 0 ? soft(Tr::ld(x[e.id[j]]), c2, top_c) * inv_sum : 0.f;
+    own[j] = e.id[j] >= 0 ? soft(Tr::ld(x[e.id[j]]), c2, top) * inv_sum : 0.f;
   __syncthreads();
   const float scale = factor * inv_sum;
   each([&](int c, const Words<S>& w) {
     if (c >= whole) return;
     Pack<S> o;
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) o.v[j] = Tr::st(scale * soft(element<Tr>(w, j), c2, top_c));
+    for (int j = 0; j < kPack; ++j) o.v[j] = Tr::st(scale * soft(element<Tr>(w, j), c2, top));
     *reinterpret_cast<Pack<S>*>(back + c) = o;
   });
-  if (whole + tid < v) back[whole + tid] = Tr::st(scale * soft(rest, c2, top_c));
+  if (whole + tid < v) back[whole + tid] = Tr::st(scale * soft(rest, c2, top));
   __syncthreads();  // the stores above come before those below
   place_entries<Tr, kThreads>(a, back, e, own, factor, 0, v);
 }

@@ -1,0 +1,161 @@
+"""The transformer ops where their numbers or sizes lie far out: logits around
+a large offset or at a mask's value, the longest rows, the most rows."""
+import math
+
+import pytest
+import torch
+
+import tensorflow_musa_extension_amd as tfma
+from test_gpu_transformer import DT, U, check, gen
+
+pytestmark = pytest.mark.gpu
+ops = tfma.raw_ops
+
+
+# ---------------------------------------------------------------------------
+# Distillation.  With the row's maxima subtracted first,
+#   loss = w T sum_j p_j ((t_j - max t) - (x_j - max x) - T (ln S_t - ln S_x)),
+# so nothing is as large as the logits themselves, and the bounds below count
+# roundings (units of U) of the differences alone.
+# ---------------------------------------------------------------------------
+def distill_bounds(logits, ids, teacher, w, t):
+    """(loss, gradient, their bounds) in float64; finite logits, and at least
+    one entry in every row."""
+    v, k = logits.shape[-1], ids.shape[-1]
+    s, w = logits.double(), w.double()
+    s = s - s.amax(-1, keepdim=True)
+    d = s / t
+    q = d.exp()
+    total = q.sum(-1, keepdim=True)
+    q = q / total
+    there = (ids >= 0) & (ids < v)
+    at = torch.where(there, ids.long(), 0)
+    r = torch.where(there, teacher.double(), -math.inf)
+    r = r - r.amax(-1, keepdim=True)
+    p = (r / t).exp()
+    mass = p.sum(-1, keepdim=True)
+    p = p / mass
+    ln_x, ln_t = total.log(), mass.log()
+    r = torch.where(there, r, 0.0)
+    x = torch.gather(s, -1, at)
+    gap = t * (ln_t - ln_x)
+    term = r - x - gap
+    loss = w * t * (p * term).sum(-1)
+    back = q.scatter_add(-1, at, -p) * (t * w)[:, None]
+    # Elements that one thread adds after the other, and the tree above it.
+    n = (v / 64 if v <= 2048 else 225 + v / 1024) + 24
+    # A weight is e^a with an argument of at most four roundings, six more
+    # for the exponential; relative, of the sums and of p.
+    e_x = (q * (4 * torch.where(q > 0, d.abs(), 0.0) + 6)).sum(-1, keepdim=True) + n
+    one = 4 * r.abs() / t + 6
+    e_t = (p * one).sum(-1, keepdim=True) + k / 64 + 16
+    e_p = one + e_t + 2
+    e_gap = t * (e_x + e_t + 4 * (ln_x.abs() + ln_t.abs())) + 4 * gap.abs()
+    e_term = 3 * (r.abs() + x.abs()) + e_gap + term.abs() * (e_p + k / 64 + 18)
+    el = w * t * (p * e_term).sum(-1) * U + 4 * U * loss.abs()
+    e_q = q * (4 * torch.where(q > 0, d.abs(), 0.0) + 16 + e_x)
+    # Weights below the smallest normal number may be 0.
+    eb = (t * w)[:, None] * (e_q.scatter_add(-1, at, p * (e_p + k + 4)) * U + 1.2e-38)
+    return loss.float().double(), back, el, eb
+
+
+@pytest.mark.parametrize("t", [1.0, 3.0, 0.7])
+@pytest.mark.parametrize("offset", [0.0, 100.0, 1e3, -1e4, 3e4])
+def test_distill_of_a_student_near_its_teacher(dev, offset, t):
+    """A small divergence keeps its digits wherever the logits lie."""
+    rows, v = 40, 1000
+    rn = gen(dev, 101)
+    g = torch.Generator(device=dev).manual_seed(102)
+    logits = rn(rows, v, scale=2.0) + offset
+    ids = torch.stack([torch.randperm(v, generator=g, device=dev) for _ in range(rows)])
+    near = torch.gather(logits, -1, ids).double() + 0.07 * rn(rows, v).double()
+    w = 0.5 + rn(rows).abs()
+    for teacher in (near.float(), (near - offset).float()):
+        loss, back, el, eb = distill_bounds(logits, ids, teacher, w, t)
+        assert bool((el < 0.05 * loss).all())  # the bound sees the loss's digits
+        got = ops.MusaTopKDistillation(logits, ids, teacher, row_weights=w, temperature=t)
+        check(got.loss, loss, el, "loss", torch.float32)
+        check(got.backprop, back, eb, "backprop", torch.float32)
+
+
+@pytest.mark.parametrize("t", [1.0, 3.0])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,v,k", [(5, 100, 9), (3, 3000, 70), (4, 8003, 20), (3, 20001, 9),
+                                      (2, 50304, 64), (2, 70000, 33)])
+def test_distill_around_an_offset(dev, rows, v, k, dtype, t):
+    """Every width's kernel with logits around 1000."""
+    rn = gen(dev, 103)
+    g = torch.Generator(device=dev).manual_seed(104)
+    logits = (rn(rows, v, scale=30.0) + 1000).to(DT[dtype])
+    ids = torch.randint(0, v, (rows, k), generator=g, device=dev)
+    teacher, w = rn(rows, k, scale=3.0, dtype=DT[dtype]), 0.5 + rn(rows).abs()
+    loss, back, el, eb = distill_bounds(logits, ids, teacher, w, t)
+    got = ops.MusaTopKDistillation(logits, ids, teacher, row_weights=w, temperature=t)
+    check(got.loss, loss, el, "loss", torch.float32)
+    check(got.backprop, back, eb, "backprop", DT[dtype])
+
+
+# Masks that programs use, and the type's own lowest and largest.
+MASKS = {"f32": [-1e4, -1e9, -1e30, "min", 1e30, "max"],
+         "bf16": [-1e4, -1e9, -1e30, "min", 1e30, "max"], "f16": [-1e4, "min", "max"]}
+
+
+@pytest.mark.parametrize("t", [1.0, 2.0, 3.0, 0.5])
+@pytest.mark.parametrize("v", [100, 8003, 50304, 70000])
+@pytest.mark.parametrize("dtype,value", [(d, m) for d in MASKS for m in MASKS[d]])
+def test_distill_of_finite_masks(dev, dtype, value, v, t):
+    """Rows that hold one finite value everywhere are uniform, whatever the
+    value; rows that hold it in half of their places keep the other half's
+    digits (and, where an entry lies on a mask, a loss as large as the mask)."""
+    dt, rows, k = DT[dtype], 6, 12
+    value = getattr(torch.finfo(dt), value) if isinstance(value, str) else value
+    rn = gen(dev, 105)
+    g = torch.Generator(device=dev).manual_seed(106)
+    logits = rn(rows, v, scale=3.0, dtype=dt)
+    ids = torch.randint(0, v, (rows, k), generator=g, device=dev)
+    logits[:3] = value
+    logits[3:, : v // 2] = value
+    ids[3] = v - 1 - torch.arange(k, device=dev)  # none on the mask
+    teacher, w = rn(rows, k, scale=3.0), 0.5 + rn(rows).abs()
+    loss, back, el, eb = distill_bounds(logits, ids, teacher, w, t)
+    got = ops.MusaTopKDistillation(logits, ids, teacher, row_weights=w, temperature=t)
+    check(got.loss, loss, el, "loss", torch.float32)
+    check(got.backprop, back, eb, "backprop", dt)
+
+
+@pytest.mark.parametrize("t", [0.5, 0.25, 2.0])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_distill_of_a_finitely_masked_teacher(dev, dtype, t):
+    """An entry at the type's lowest value is there: it has no weight beside
+    larger ones, and a row of such entries is uniform."""
+    dt, rows, v, k = DT[dtype], 4, 300, 8
+    rn = gen(dev, 107)
+    logits, teacher, w = rn(rows, v, dtype=dt), rn(rows, k, dtype=dt), 0.5 + rn(rows).abs()
+    ids = torch.arange(rows * k, device=dev).reshape(rows, k)
+    low = torch.finfo(dt).min
+    teacher[0] = low
+    teacher[1, 3:] = low
+    teacher[2] = -low
+    teacher[3, 0] = -low
+    loss, back, el, eb = distill_bounds(logits, ids, teacher, w, t)
+    got = ops.MusaTopKDistillation(logits, ids, teacher, row_weights=w, temperature=t)
+    check(got.loss, loss, el, "loss", torch.float32)
+    check(got.backprop, back, eb, "backprop", dt)
+
+
+@pytest.mark.parametrize("t", [1e-3, 1e-30, 1e-39, 1e-45])
+def test_distill_at_the_smallest_temperatures(dev, t):
+    """The softmax is its maximum's place; no 0 meets an infinity."""
+    v = 500
+    logits = gen(dev, 108)(2, v)
+    logits[:, 7] = 20
+    ids = torch.tensor([[7, 3], [7, 9]], device=dev)
+    teacher = torch.tensor([[3.0, -8.0], [-8.0, 3.0]], device=dev)
+    got = ops.MusaTopKDistillation(logits, ids, teacher, temperature=t)
+    # The teacher's place is the student's in one row and 20 - x[9] below its
+    # largest in the other: loss T (20 - x[9]).
+    want = float(torch.tensor(t)) * (20 - float(logits[1, 9]))
+    assert float(got.loss[0]) == 0 and abs(float(got.loss[1]) - want) <= 4 * U * want + 2.0 ** -149
+    back = torch.zeros(2, v, device=dev)
+    back[1, 7], back[1, 9] = float(torch.tensor(t)), -float(torch.tensor(t))
+    assert torch.equal(got.backprop, back)

@@ -1556,8 +1556,9 @@ struct Arg {
   const char* name;
 };
 
-// No output lies over an input or another output, except that an output may
-// be one of `in_place` itself (same memory, size and type).
+// No output lies over an input or another output, except that each of them may
+// be one of `in_place` itself (same memory, size and type): elements that are
+// read by the thread that then writes them.
 int check_overlap(const char* op, std::initializer_list<Arg> outs, std::initializer_list<Arg> ins,
                   std::initializer_list<Arg> in_place, TFMA_Status* st) {
   for (const Arg* po = outs.begin(); po != outs.end(); ++po) {
@@ -1572,7 +1573,8 @@ int check_overlap(const char* op, std::initializer_list<Arg> outs, std::initiali
         return set_status(st, TFMA_INVALID_ARGUMENT, "%s: %s overlaps %s", op, o.name, in.name);
     for (const Arg& in : in_place)
       if (in.t && overlap(o.t, in.t) &&
-          (in.t->data != o.t->data || in.t->dtype != o.t->dtype))
+          (in.t->data != o.t->data || in.t->dtype != o.t->dtype ||
+           tensor_bytes(in.t) != tensor_bytes(o.t)))
         return set_status(st, TFMA_INVALID_ARGUMENT, "%s: %s overlaps %s in part", op, o.name,
                           in.name);
   }
@@ -1651,8 +1653,15 @@ int rms_norm_impl(const char* op, void* stream, const TFMA_Tensor* x, const TFMA
   TFMA_Tensor* per_row = scale ? scale : rstd;
   if (const int rc = check_arg(op, {per_row, scale ? "scale" : "rstd"}, TFMA_FLOAT, {}, x, lead, st))
     return rc;
-  if (const int rc = check_overlap(op, {{y, "y"}, {sum, "sum"}, {per_row, scale ? "scale" : "rstd"}},
-                                   {{gamma, "gamma"}}, {{x, "x"}, {residual, "residual"}}, st))
+  // y and sum may replace x and residual.  rstd and scale may not, of any size:
+  // a row's is written while other rows are still read.
+  const Arg statistic = {per_row, scale ? "scale" : "rstd"};
+  if (const int rc = check_overlap(op, {{y, "y"}, {sum, "sum"}, statistic}, {{gamma, "gamma"}}, {}, st))
+    return rc;
+  if (const int rc = check_overlap(op, {{y, "y"}, {sum, "sum"}}, {},
+                                   {{x, "x"}, {residual, "residual"}}, st))
+    return rc;
+  if (const int rc = check_overlap(op, {statistic}, {{x, "x"}, {residual, "residual"}}, {}, st))
     return rc;
   a.epsilon = epsilon;
   a.x = x->data;
@@ -1862,10 +1871,14 @@ int TFMA_MusaAddRmsNormGrad(void* stream, const TFMA_Tensor* y_backprop, const T
                                status))
     return rc;
   if (const int rc = check_overlap(op, {{x_backprop, "x_backprop"}, {gamma_backprop, "gamma_backprop"}},
-                                   {{gamma, "gamma"}, {rstd, "rstd"}},
-                                   {{y_backprop, "y_backprop"}, {sum, "sum"},
-                                    {sum_backprop, "sum_backprop"}},
-                                   status))
+                                   {{gamma, "gamma"}, {rstd, "rstd"}}, {}, status))
+    return rc;
+  // x_backprop may replace one of the inputs of its shape; gamma_backprop, which
+  // is written while other rows are still read, may not.
+  const std::initializer_list<Arg> rows_in = {
+      {y_backprop, "y_backprop"}, {sum, "sum"}, {sum_backprop, "sum_backprop"}};
+  if (const int rc = check_overlap(op, {{x_backprop, "x_backprop"}}, {}, rows_in, status)) return rc;
+  if (const int rc = check_overlap(op, {{gamma_backprop, "gamma_backprop"}}, rows_in, {}, status))
     return rc;
   if (const int rc = check_workspace(op, workspace, workspace_bytes,
                                      RmsNormGradWorkspaceBytes(a.rows, a.c), status))

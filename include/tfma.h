@@ -388,8 +388,9 @@ int TFMA_MusaLinear(void* stream, const TFMA_Tensor* x, const TFMA_Tensor* w,
  * [N, K] with w_scale FLOAT [N]; z = x_scale w_scale (x w^T) + bias.  y, bias
  * and residual are all HALF or all BFLOAT16 (the matrix cores add 8-bit
  * products to about 13 bits of the largest, which a FLOAT result would show).
- * K is a multiple of 16 and x and w are 16-byte aligned.  The workspace is TFMA_MusaLinearWorkspaceBytes with transpose_b
- * = 1. */
+ * K is a multiple of 16, at most 2^23 (UNIMPLEMENTED past it, from the size
+ * query too), and x and w are 16-byte aligned.  The workspace is
+ * TFMA_MusaLinearWorkspaceBytes with transpose_b = 1. */
 int TFMA_MusaLinearQuantized(void* stream, const TFMA_Tensor* x, const TFMA_Tensor* x_scale,
                              const TFMA_Tensor* w, const TFMA_Tensor* w_scale,
                              const TFMA_Tensor* bias, const TFMA_Tensor* residual,

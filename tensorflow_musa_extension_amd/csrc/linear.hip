@@ -634,6 +634,9 @@ template <int kTM_, int kTN_, int kWavesM_, int kWavesN_, int kSlots_, int kRegi
           bool kTurned_ = false>
 struct Config {
   static constexpr bool kTurned = kTurned_;
+  // A tile's longest rows end below DirectTile::kOutside, which no sum of an
+  // offset and the way down from it then passes by 2^32 either.
+  static_assert((kTM_ > kTN_ ? kTM_ : kTN_) * kLinear8MaxK <= int64_t(1) << 31, "offsets in 31 bits");
   static constexpr int kTM = kTM_, kTN = kTN_, kWavesM = kWavesM_, kWavesN = kWavesN_,
                        kSlots = kSlots_, kWaves = kWavesM * kWavesN;
   static constexpr int kFM = kTM / kWavesM / 16, kFN = kTN / kWavesN / 16;  // fragments of a wave

@@ -1714,6 +1714,10 @@ int linear_geometry(const char* op, const TFMA_Tensor* x, const TFMA_Tensor* w, 
                       shape_str(w).c_str());
   if (*k >= (int64_t(1) << 30) || *n >= (int64_t(1) << 30))
     return set_status(st, TFMA_UNIMPLEMENTED, "%s: dimension too large", op);
+  if (x->dtype == TFMA_FLOAT8_E4M3FN && *k > kLinear8MaxK)
+    return set_status(st, TFMA_UNIMPLEMENTED,
+                      "%s: the inner dimension of 8-bit operands must be at most %lld, got %lld", op,
+                      static_cast<long long>(kLinear8MaxK), static_cast<long long>(*k));
   if ((!x->data && *m * *k > 0) || (!w->data && *k * *n > 0))
     return set_status(st, TFMA_INVALID_ARGUMENT, "%s: null input", op);
   return TFMA_OK;

@@ -342,8 +342,10 @@ size_t LinearWorkspaceBytes(DType t, bool e4m3, const GemmShape& s, const void* 
 hipError_t LaunchLinear(DType t, const GemmShape& s, const void* a, const void* b,
                         const LinearEpilogue& e, void* workspace, size_t workspace_bytes,
                         hipStream_t stream);
-// 8-bit (e4m3) operands, both with k contiguous and k a multiple of 16;
-// t: C's type, half or bfloat16.
+// 8-bit (e4m3) operands, both with k contiguous and k a multiple of 16, at most
+// kLinear8MaxK: these have no other kernel, and the offsets of a tile's rows,
+// of which there are up to 256, are 31 bits.  t: C's type, half or bfloat16.
+constexpr int64_t kLinear8MaxK = int64_t(1) << 23;
 hipError_t LaunchLinear8(DType t, const GemmShape& s, const void* a, const void* b,
                          const LinearEpilogue& e, void* workspace, size_t workspace_bytes,
                         hipStream_t stream);

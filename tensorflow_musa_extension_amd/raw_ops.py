@@ -566,8 +566,9 @@ def MusaLinear(x, w, bias=None, residual=None, activation="", transpose_b=False,
 def MusaLinearQuantized(x, x_scale, w, w_scale, bias=None, residual=None, activation="",
                         out_type=torch.bfloat16, workspace=None, out=None):
     """MusaLinear of float8_e4m3fn operands: x [..., K] with a float32 scale
-    per row, w [N, K] with one per output column.  Returns y in out_type
-    (bfloat16 or float16, the type of bias and residual too)."""
+    per row, w [N, K] with one per output column, K a multiple of 16 up to
+    2^23.  Returns y in out_type (bfloat16 or float16, the type of bias and
+    residual too)."""
     if out is None:
         out = torch.empty(_linear_shape(x, w, True), dtype=out_type, device=x.device)
     dx, dxs, dw, dws, dy = (_d(x, "x"), _d(x_scale, "x_scale"), _d(w, "w"),

@@ -159,3 +159,38 @@ def test_distill_at_the_smallest_temperatures(dev, t):
     back = torch.zeros(2, v, device=dev)
     back[1, 7], back[1, 9] = float(torch.tensor(t)), -float(torch.tensor(t))
     assert torch.equal(got.backprop, back)
+
+
+# ---------------------------------------------------------------------------
+# Products
+# ---------------------------------------------------------------------------
+def sparse_places(dev, k, n, seed):
+    """n places of [0, k): the first, the last, those around every quarter and
+    others as they fall."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    fixed = [q * k // 4 + d for q in range(1, 4) for d in (-1, 0)] + [0, 1, k - 2, k - 1]
+    rest = torch.randint(0, k, (n - len(fixed),), generator=g, device=dev)
+    return torch.cat([torch.tensor(fixed, device=dev), rest]).unique()
+
+
+@pytest.mark.parametrize("tile", [0, 1, 2, 3, None])
+def test_linear_quantized_longest_rows(dev, tune, tile):
+    """Rows of 8 MiB, 256 of a tile: their offsets pass 2^31 by nothing.  x is
+    zero but for some hundred whole numbers a row, w is -1, 0 and 1: sums that
+    every order of them holds exactly."""
+    m, k, n = 256, 1 << 23, 256
+    if tile is not None:
+        tune("linear_tile", tile)
+        tune("linear_splits", 8)
+    g = torch.Generator(device=dev).manual_seed(110)
+    at = sparse_places(dev, k, 200, 111)
+    some = torch.randint(-2, 3, (m, at.numel()), generator=g, device=dev).float()
+    x = torch.zeros(m, k, dtype=torch.uint8, device=dev)
+    x[:, at] = some.to(torch.float8_e4m3fn).view(torch.uint8)
+    w = torch.randint(0, 3, (n, k), generator=g, device=dev, dtype=torch.uint8)
+    w = torch.where(w == 2, 0xB8, w * 0x38).to(torch.uint8).view(torch.float8_e4m3fn)
+    one = torch.ones(n, device=dev)
+    got = ops.MusaLinearQuantized(x.view(torch.float8_e4m3fn), one, w, one, out_type=torch.float16)
+    want = some.double() @ w.view(torch.uint8)[:, at].view(torch.float8_e4m3fn).double().T
+    assert float(want.std()) > 5
+    assert torch.equal(got.double(), want)

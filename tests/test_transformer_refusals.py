@@ -39,3 +39,22 @@ def test_gamma_backprop_is_no_input(rows, c, which):
                      T(3, (rows,)), a["sum_backprop"], T(4, (rows, c)), over,
                      ctypes.c_void_p(A + 9 * GAP), 1 << 30)
     assert (code, msg) == (INV, f"MusaAddRmsNormGrad: gamma_backprop overlaps {which}")
+
+
+@pytest.mark.parametrize("k", [(1 << 23) + 16, 17825792, 1 << 25, (1 << 30) - 16])
+def test_8_bit_rows_past_the_tiles_offsets(k):
+    """Rows whose 256 of a tile pass 2^31 bytes."""
+    x, w = T(0, (1, k), Q), T(20, (128, k), Q)
+    want = ("MusaLinearQuantized: the inner dimension of 8-bit operands must be at most 8388608, "
+            f"got {k}")
+    code, msg = call("TFMA_MusaLinearQuantized", None, x, T(60, (1,)), w, T(61, (128,)), None, None,
+                     b"", T(62, (1, 128), B), ctypes.c_void_p(A + 70 * GAP), 1 << 30)
+    assert (code, msg) == (UNI, want)
+    code, msg, _ = size("TFMA_MusaLinearWorkspaceBytes", x, w, 1)
+    assert (code, msg) == (UNI, want.replace("Quantized", ""))
+
+
+def test_8_bit_rows_as_long_as_the_tiles_offsets():
+    code, _, need = size("TFMA_MusaLinearWorkspaceBytes", T(0, (64, 1 << 23), Q),
+                         T(20, (128, 1 << 23), Q), 1)
+    assert code == _lib.OK and need > 0

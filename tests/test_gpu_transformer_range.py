@@ -194,3 +194,31 @@ def test_linear_quantized_longest_rows(dev, tune, tile):
     want = some.double() @ w.view(torch.uint8)[:, at].view(torch.float8_e4m3fn).double().T
     assert float(want.std()) > 5
     assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("tb", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_linear_of_rows_over_4_mib(dev, dtype, tb):
+    """The kernel of the longest rows, with operands of more than 2^31 bytes,
+    at whole numbers whose sums are exact."""
+    dt = DT[dtype]
+    long = (1 << 22) // dt.itemsize + 72
+    g = torch.Generator(device=dev).manual_seed(112)
+    if tb:  # both operands' rows, and a long sum
+        m, k, n = 520, long, 520
+        at = sparse_places(dev, k, 100, 113)
+        some = torch.randint(-2, 3, (m, at.numel()), generator=g, device=dev).to(dt)
+        x = torch.zeros(m, k, dtype=dt, device=dev)
+        x[:, at] = some
+        w = torch.randint(-1, 2, (n, k), generator=g, device=dev, dtype=torch.int8).to(dt)
+        want = some.double() @ w[:, at].double().T
+    else:  # w's rows
+        m, k, n = 40, 520, long
+        x = torch.randint(-2, 3, (m, k), generator=g, device=dev).to(dt)
+        x[:, torch.rand(k, generator=g, device=dev) < 0.8] = 0
+        w = torch.randint(-1, 2, (k, n), generator=g, device=dev, dtype=torch.int8).to(dt)
+        want = (x.float() @ w.float()).double()  # whole numbers below 2^24
+    assert float(want.std()) > 5 and float(want.abs().max()) <= 256
+    got = ops.MusaLinear(x, w, transpose_b=tb).y
+    assert ops.last_kernel_name() == "tfma_linear"
+    assert torch.equal(got.double(), want)

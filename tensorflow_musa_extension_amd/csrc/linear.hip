@@ -1029,7 +1029,13 @@ __global__ __launch_bounds__(kWaves * 64) void few_rows_kernel(GemmShape s, int 
 //   workgroups, 14.9 / 12.2; f32 16 x 2048 x 2048 16.5 / 13.6;
 //   B [n, k] bf16, up to 16 rows: 16 x 1024 x 1024 5.9 / 8.9, 16 x 4096 x 4096
 //   10.6 / 11.9, 16 x 4096 x 8192, whose read the loads to LDS carry better,
-//   21.6 / 15.4 (f32 16 x 4096 x 4096 20.3 / 25.7); 32 x 2048 x 8192 15.5 / 11.9.
+//   21.6 / 15.4 (f32 16 x 4096 x 4096 20.3 / 25.7); 32 x 2048 x 8192 15.5 / 11.9;
+//   B [n, k] e4m3, whose turn takes 2048 k and whose reads of A count, one
+//   round of workgroups and less than a turn: 1 x 512 x 4096 5.3 / 6.4, 1 x 1536 x
+//   1536 8.0 / 10.0, 4 x 1024 x 4096 7.1 / 8.3, 16 x 256 x 2048 4.7 / 5.4, 16 x
+//   512 x 4096 6.4 / 6.4; past that 1 x 512 x 8192 7.7 / 6.5, 4 x 2048 x 2048 10.2
+//   / 8.7, 16 x 1024 x 1024 8.8 / 8.2, 1 x 2048 x 8192 17.8 / 9.9, 16 x 4096 x 8192
+//   47.6 / 13.3.
 constexpr int kFewRows = 32;
 constexpr int kFewWaves = 16;
 
@@ -1039,6 +1045,7 @@ int few_step(bool b_kc, int esize) { return b_kc ? kRowBytes / esize : (esize ==
 bool few_rows(const GemmShape& s, bool direct, int esize) {
   if (!s.a_kc || s.m > kFewRows) return false;
   if (!direct) return true;
+  if (esize == 1) return s.m <= 16 && s.n <= 4096 && s.k <= (s.m <= 4 ? 1536 : 512);
   const int64_t bytes = s.k * s.n * esize, turn = int64_t(kFewWaves) * few_step(s.b_kc, esize);
   const int64_t turns = (s.k + turn - 1) / turn;
   if (s.b_kc) return s.m <= 16 && s.k <= 4096 && bytes <= (int64_t(esize == 4 ? 72 : 48) << 20);
@@ -1245,8 +1252,9 @@ hipError_t launch(const GemmShape& s, DType t, const void* a, const void* b, con
       const FewPlan p = plan_few(kBKC, s, kE);
       if (sums_bytes(s, p.splits) > ws.bytes) return hipErrorInvalidValue;
       if constexpr (kBKC) {
-        return p.nj == 2 ? launch_few<Op, Tr, true, 2>(s, a, b, e, ws.at, p.splits, stream)
-                         : launch_few<Op, Tr, true, 1>(s, a, b, e, ws.at, p.splits, stream);
+        if constexpr (kE > 1)  // e4m3: one round of workgroups
+          if (p.nj == 2) return launch_few<Op, Tr, true, 2>(s, a, b, e, ws.at, p.splits, stream);
+        return launch_few<Op, Tr, true, 1>(s, a, b, e, ws.at, p.splits, stream);
       } else {
         return launch_few<Op, Tr, false, 4>(s, a, b, e, ws.at, p.splits, stream);
       }

@@ -222,3 +222,26 @@ def test_linear_of_rows_over_4_mib(dev, dtype, tb):
     got = ops.MusaLinear(x, w, transpose_b=tb).y
     assert ops.last_kernel_name() == "tfma_linear"
     assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("shape,few", [
+    ((1, 16, 1), True), ((1, 512, 4096), True), ((4, 1536, 300), True), ((3, 1040, 70), True),
+    ((16, 512, 4096), True), ((13, 400, 75), True), ((5, 16, 4095), True),
+    ((1, 512, 4097), False), ((4, 1552, 300), False), ((5, 528, 70), False), ((16, 1024, 1024), False),
+    ((1, 2048, 8192), False), ((16, 2048, 2048), False), ((16, 4096, 4096), False),
+    ((16, 4096, 8192), False), ((9, 4096, 72), False)])
+def test_linear_quantized_of_few_tokens(dev, shape, few):
+    """Either kernel on its side of the rule, at whole numbers whose sums are
+    exact."""
+    m, k, n = shape
+    g = torch.Generator(device=dev).manual_seed(114)
+    x = torch.randint(-2, 3, (m, k), generator=g, device=dev)
+    x[torch.rand(m, k, generator=g, device=dev) < max(0.0, 1 - 200 / k)] = 0
+    w = torch.randint(-1, 2, (n, k), generator=g, device=dev)
+    xs = 2.0 ** torch.randint(-2, 3, (m,), generator=g, device=dev)
+    ws = 2.0 ** torch.randint(-2, 3, (n,), generator=g, device=dev)
+    f8 = torch.float8_e4m3fn
+    got = ops.MusaLinearQuantized(x.to(f8), xs, w.to(f8), ws, out_type=torch.float16)
+    assert (ops.last_kernel_name() == "tfma_linear_few") == few
+    want = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
+    assert torch.equal(got.double(), want)

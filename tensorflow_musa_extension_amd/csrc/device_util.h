@@ -11,6 +11,22 @@
 namespace tfma {
 
 // ---------------------------------------------------------------------------
+// Grids of many workgroups.  A grid's threads along one dimension are counted
+// in 32 bits, and a launch of more wraps around without an error (2^24 + 5
+// workgroups of 256 threads run 5 of them).  many_groups lays `groups`
+// workgroups out in two dimensions; those past `groups` return at once.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kGroupsAcross = 1u << 20;  // of up to 1024 threads
+constexpr int64_t kMostGroups = int64_t(kGroupsAcross) * 65535;
+inline dim3 many_groups(int64_t groups) {
+  if (groups <= kGroupsAcross) return dim3(static_cast<uint32_t>(groups));
+  return dim3(kGroupsAcross, static_cast<uint32_t>((groups + kGroupsAcross - 1) / kGroupsAcross));
+}
+__device__ inline int64_t group_of_many() {
+  return int64_t(blockIdx.y) * kGroupsAcross + blockIdx.x;
+}
+
+// ---------------------------------------------------------------------------
 // Type traits.  S = storage type in HBM, C = compute type in registers.
 // `rnd` rounds a compute value to the storage precision and back; TF's CPU
 // kernels (Eigen) evaluate half/bfloat16 arithmetic as float and round to the

@@ -189,7 +189,8 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
   const Entries e = {reinterpret_cast<int32_t*>(dyn), dyn + a.k, dyn + 2 * a.k};
   float* own = dyn + 3 * a.k;
   const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const int64_t row = group_of_many();
+  if (row >= a.rows) return;
   const S* x = static_cast<const S*>(a.logits) + row * a.v;
   const int v = static_cast<int>(a.v), whole = v & ~(kPack - 1);
   constexpr int kHeld = kPacks > 0 ? kPacks : 1;
@@ -268,10 +269,9 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
 
 template <class Tr, int kThreads, int kPacks>
 hipError_t launch(const DistillArgs& a, hipStream_t stream) {
-  if (a.rows >= (int64_t(1) << 31)) return hipErrorInvalidConfiguration;
-  TFMA_LAUNCH("tfma_distill", (distill_kernel<Tr, kThreads, kPacks>),
-              dim3(static_cast<uint32_t>(a.rows)), dim3(kThreads), 4 * a.k * sizeof(float), stream,
-              a);
+  if (a.rows > kMostGroups) return hipErrorInvalidConfiguration;
+  TFMA_LAUNCH("tfma_distill", (distill_kernel<Tr, kThreads, kPacks>), many_groups(a.rows),
+              dim3(kThreads), 4 * a.k * sizeof(float), stream, a);
   return hipGetLastError();
 }
 

@@ -814,7 +814,7 @@ template <class Tr>
 __global__ __launch_bounds__(256) void join_kernel(int64_t m, int64_t n, int splits,
                                                    const float* partial, LinearEpilogue e) {
   const int64_t per_row = (n + 7) / 8;
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t i = group_of_many() * 256 + threadIdx.x;
   if (i >= m * per_row) return;
   const int64_t row = i / per_row, col = i % per_row * 8;
   const float* p = partial + row * n + col;
@@ -840,8 +840,8 @@ template <class Tr>
 hipError_t launch_join(const GemmShape& s, int splits, const void* workspace, const LinearEpilogue& e,
                        hipStream_t stream) {
   const int64_t groups = (s.m * ((s.n + 7) / 8) + 255) / 256;
-  TFMA_LAUNCH("tfma_linear_join", join_kernel<Tr>, dim3(static_cast<uint32_t>(groups)), dim3(256), 0,
-              stream, s.m, s.n, splits, static_cast<const float*>(workspace), e);
+  TFMA_LAUNCH("tfma_linear_join", join_kernel<Tr>, many_groups(groups), dim3(256), 0, stream, s.m,
+              s.n, splits, static_cast<const float*>(workspace), e);
   return hipGetLastError();
 }
 
@@ -922,8 +922,10 @@ __global__ __launch_bounds__(kWaves * 64) void few_rows_kernel(GemmShape s, int 
   const S* a = static_cast<const S*>(a_);
   const S* b = static_cast<const S*>(b_);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int tile = blockIdx.x / splits, split = blockIdx.x % splits;
+  const uint32_t group = static_cast<uint32_t>(group_of_many());
+  const int tile = group / splits, split = group % splits;
   const int64_t n0 = int64_t(tile) * kCols;
+  if (n0 >= s.n) return;
   f32x4 acc[kMT][kNJ] = {};
   const int64_t k_end = int64_t(split + 1) * steps * kBK < s.k ? int64_t(split + 1) * steps * kBK : s.k;
   for (int64_t k = (int64_t(split) * steps + wave) * kBK; k < k_end; k += kWaves * kBK) {
@@ -1081,7 +1083,7 @@ hipError_t launch_few(const GemmShape& s, const void* a, const void* b, const Li
   const int bk = few_step(kBKC, sizeof(typename Op::S));
   const int64_t tiles = (s.n + 16 * kNJ - 1) / (16 * kNJ), all = (s.k + bk - 1) / bk;
   const int steps = static_cast<int>((all + splits - 1) / splits);
-  const dim3 grid(static_cast<uint32_t>(tiles * splits)), block(kFewWaves * 64);
+  const dim3 grid = many_groups(tiles * splits), block(kFewWaves * 64);
   float* partial = static_cast<float*>(workspace);
   constexpr bool kWide = sizeof(typename Op::S) > 1;  // e4m3 operands never need 32 rows
   if (!kWide || s.m <= 16)
@@ -1156,7 +1158,7 @@ struct PadArgs {
   const void* from[2];
   void* to[2];
   int64_t rows[2], cols[2], ld[2];
-  uint32_t groups0;  // workgroups of the first operand
+  uint32_t groups0, groups;  // workgroups of the first operand, and of both
 };
 __host__ __device__ inline uint32_t pad_pieces(int64_t ld, int esize) {
   return static_cast<uint32_t>((ld * esize + 1023) / 1024);
@@ -1164,8 +1166,10 @@ __host__ __device__ inline uint32_t pad_pieces(int64_t ld, int esize) {
 template <typename S>
 __global__ __launch_bounds__(256) void pad_kernel(PadArgs p) {
   constexpr int kN = 16 / static_cast<int>(sizeof(S));
-  const int which = blockIdx.x < p.groups0 ? 0 : 1;
-  const uint32_t piece = (blockIdx.x - (which ? p.groups0 : 0)) * 4 + (threadIdx.x >> 6);
+  const uint32_t group = static_cast<uint32_t>(group_of_many());
+  if (group >= p.groups) return;
+  const int which = group < p.groups0 ? 0 : 1;
+  const uint32_t piece = (group - (which ? p.groups0 : 0)) * 4 + (threadIdx.x >> 6);
   const uint32_t per_row = pad_pieces(p.ld[which], sizeof(S));
   const int64_t row = piece / per_row;
   const int64_t c = (int64_t(piece % per_row) * 64 + (threadIdx.x & 63)) * kN;
@@ -1227,8 +1231,8 @@ hipError_t launch_pad(const GemmShape& s, const Padding& p, const void*& a, cons
   if (groups == 0) return hipSuccess;
   if (groups >= (int64_t(1) << 30)) return hipErrorInvalidConfiguration;
   args.groups0 = static_cast<uint32_t>(groups0);
-  TFMA_LAUNCH("tfma_linear_pad", pad_kernel<S>, dim3(static_cast<uint32_t>(groups)), dim3(256), 0,
-              stream, args);
+  args.groups = static_cast<uint32_t>(groups);
+  TFMA_LAUNCH("tfma_linear_pad", pad_kernel<S>, many_groups(groups), dim3(256), 0, stream, args);
   return hipGetLastError();
 }
 
@@ -1290,7 +1294,7 @@ hipError_t launch(const GemmShape& s, DType t, const void* a, const void* b, con
     }
     // Rows of more than 4 MiB.
     const int64_t tiles = ((s.m + kTile - 1) / kTile) * ((s.n + kTile - 1) / kTile);
-    if (tiles >= (int64_t(1) << 31)) return hipErrorInvalidConfiguration;
+    if (tiles * kThreads > UINT32_MAX) return hipErrorInvalidConfiguration;
     TFMA_LAUNCH("tfma_linear", (linear_kernel<Op, Tr, kAKC, kBKC>),
                 dim3(static_cast<uint32_t>(tiles)), dim3(kThreads), 0, stream, s, a, b, e);
     return hipGetLastError();

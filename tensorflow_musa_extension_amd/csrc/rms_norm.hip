@@ -119,8 +119,8 @@ template <class Tr, int kThreads, int kPacks>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void norm_kernel(RmsNormArgs a) {
   __shared__ float lds[kThreads / 64];
   constexpr int kRows = kThreads < 256 ? 256 / kThreads : 1;
-  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kThreads;
-  if (row >= a.rows) return;  // whole waves; workgroups of one row never
+  const int64_t row = group_of_many() * kRows + threadIdx.x / kThreads;
+  if (row >= a.rows) return;  // whole waves, and whole workgroups of one row
   const int tid = threadIdx.x % kThreads;
   const int n = static_cast<int>(a.c);
   const int64_t at = row * a.c;
@@ -187,7 +187,8 @@ template <class Tr>
 __global__ __launch_bounds__(1024) void norm_long_kernel(RmsNormArgs a) {
   constexpr int kThreads = 1024;
   __shared__ float lds[kThreads / 64];
-  const int64_t row = blockIdx.x;
+  const int64_t row = group_of_many();
+  if (row >= a.rows) return;
   const int64_t at = row * a.c;
   const int n = static_cast<int>(a.c);
   const int tid = threadIdx.x;
@@ -251,9 +252,9 @@ template <class Tr, int kThreads, int kPacks>
 hipError_t launch_norm(const RmsNormArgs& a, hipStream_t stream) {
   constexpr int kRows = kThreads < 256 ? 256 / kThreads : 1;
   const int64_t groups = (a.rows + kRows - 1) / kRows;
-  if (groups >= (int64_t(1) << 31)) return hipErrorInvalidConfiguration;
-  TFMA_LAUNCH("tfma_rms_norm", (norm_kernel<Tr, kThreads, kPacks>),
-              dim3(static_cast<uint32_t>(groups)), dim3(kRows * kThreads), 0, stream, a);
+  if (groups > kMostGroups) return hipErrorInvalidConfiguration;
+  TFMA_LAUNCH("tfma_rms_norm", (norm_kernel<Tr, kThreads, kPacks>), many_groups(groups),
+              dim3(kRows * kThreads), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -269,9 +270,9 @@ hipError_t norm_by_width(const RmsNormArgs& a, hipStream_t stream) {
   if (a.c <= 512 * 8) return launch_norm<Tr, 512, 1>(a, stream);
   if (a.c <= 1024 * 8) return launch_norm<Tr, 1024, 1>(a, stream);
   if (a.c <= 1024 * 16) return launch_norm<Tr, 1024, 2>(a, stream);
-  if (a.rows >= (int64_t(1) << 31)) return hipErrorInvalidConfiguration;
-  TFMA_LAUNCH("tfma_rms_norm_long", norm_long_kernel<Tr>, dim3(static_cast<uint32_t>(a.rows)),
-              dim3(1024), 0, stream, a);
+  if (a.rows > kMostGroups) return hipErrorInvalidConfiguration;
+  TFMA_LAUNCH("tfma_rms_norm_long", norm_long_kernel<Tr>, many_groups(a.rows), dim3(1024), 0, stream,
+              a);
   return hipGetLastError();
 }
 
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(1024) void gamma_sums_kernel(int64_t groups, int64_
                                                           const float* partial, float* out) {
   __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i = int64_t(blockIdx.x) * 64 + lane;
+  const int64_t i = group_of_many() * 64 + lane;
   float s = 0.f;
   if (i < c) {
 #pragma unroll 8
@@ -486,9 +487,8 @@ hipError_t norm_grad(const RmsNormGradArgs& a, hipStream_t stream) {
     const hipError_t e = norm_grad_by_width<Tr>(b, groups, rows_per, stream);
     if (e != hipSuccess || groups == 1) return e;
   }
-  TFMA_LAUNCH("tfma_rms_norm_dgamma", gamma_sums_kernel,
-              dim3(static_cast<uint32_t>((a.c + 63) / 64)), dim3(1024), 0, stream, groups, a.c,
-              a.partial, a.dgamma);
+  TFMA_LAUNCH("tfma_rms_norm_dgamma", gamma_sums_kernel, many_groups((a.c + 63) / 64), dim3(1024), 0,
+              stream, groups, a.c, a.partial, a.dgamma);
   return hipGetLastError();
 }
 

@@ -245,3 +245,105 @@ def test_linear_quantized_of_few_tokens(dev, shape, few):
     assert (ops.last_kernel_name() == "tfma_linear_few") == few
     want = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
     assert torch.equal(got.double(), want)
+
+
+# ---------------------------------------------------------------------------
+# More threads than a grid's dimension counts: rows of few elements (and the
+# longest rows) in numbers that take more than 2^32.
+# ---------------------------------------------------------------------------
+def some_rows(dev, rows, of_a_grid):
+    """Rows at both ends, on both sides of `of_a_grid` and in between."""
+    g = torch.Generator(device=dev).manual_seed(120)
+    some = torch.randint(0, rows, (40,), generator=g, device=dev)
+    ends = [0, 1, 19, 20, of_a_grid - 1, of_a_grid, rows - 2, rows - 1]
+    return torch.cat([torch.tensor(ends, device=dev), some])
+
+
+def test_norm_of_more_rows_than_a_grid_counts(dev):
+    rows, c = (1 << 26) + 77, 8
+    x = torch.empty(rows, c, dtype=torch.bfloat16, device=dev)
+    x.normal_(generator=torch.Generator(device=dev).manual_seed(121))
+    gamma = torch.ones(c, device=dev)
+    out = ops.MusaAddRmsNormResult(torch.full_like(x, math.nan), x,
+                                   torch.full((rows,), math.nan, device=dev))
+    ops.MusaAddRmsNorm(x, gamma, out=out)
+    assert not bool(out.rstd.isnan().any()) and not bool(out.y.isnan().any())
+    pick = some_rows(dev, rows, 1 << 26)
+    want = ops.MusaAddRmsNorm(x[pick], gamma)
+    assert torch.equal(out.y[pick], want.y) and torch.equal(out.rstd[pick], want.rstd)
+    q = ops.MusaAddRmsNormQuantizedResult(torch.zeros(rows, c, dtype=torch.float8_e4m3fn, device=dev),
+                                          out.rstd.fill_(math.nan), x)
+    ops.MusaAddRmsNormQuantized(x, gamma, out=q)
+    assert not bool(q.scale.isnan().any())
+    wq = ops.MusaAddRmsNormQuantized(x[pick], gamma)
+    assert torch.equal(q.y.view(torch.uint8)[pick], wq.y.view(torch.uint8))
+
+
+def test_norm_of_more_wide_rows_than_a_grid_counts(dev):
+    """A workgroup a row, over the input's own memory."""
+    rows, c = (1 << 24) + 77, 1032
+    x = torch.empty(rows, c, dtype=torch.bfloat16, device=dev)
+    x.normal_(generator=torch.Generator(device=dev).manual_seed(122))
+    gamma = torch.ones(c, device=dev)
+    pick = some_rows(dev, rows, 1 << 24)
+    want = ops.MusaAddRmsNorm(x[pick], gamma)
+    rstd = torch.full((rows,), math.nan, device=dev)
+    ops.MusaAddRmsNorm(x, gamma, out=ops.MusaAddRmsNormResult(x, x, rstd))
+    assert not bool(rstd.isnan().any())
+    assert torch.equal(x[pick], want.y) and torch.equal(rstd[pick], want.rstd)
+
+
+def test_norm_grad_of_the_longest_rows(dev):
+    """gamma's gradient has more columns than a grid counts."""
+    rows, c = 6, (1 << 28) + 136
+    g = torch.Generator(device=dev).manual_seed(123)
+    h = torch.empty(rows, c, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    gamma = torch.ones(c, device=dev)
+    rstd = torch.ones(rows, device=dev)
+    out = ops.MusaAddRmsNormGradResult(torch.empty_like(h), torch.full((c,), math.nan, device=dev))
+    ops.MusaAddRmsNormGrad(h, h, gamma, rstd, out=out)
+    assert not bool(out.gamma_backprop.isnan().any())
+    last = slice(c - 200, c)
+    for at in (slice(0, 200), slice(c // 2, c // 2 + 200), last):
+        want = h[:, at].double().square()
+        check(out.gamma_backprop[at], want.sum(0), want.sum(0) * (rows + 4) * U, "dgamma")
+
+
+def test_distill_of_more_rows_than_a_grid_counts(dev):
+    rows, v, k = (1 << 26) + 77, 9, 2
+    g = torch.Generator(device=dev).manual_seed(124)
+    logits = torch.empty(rows, v, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    ids = torch.randint(0, v, (rows, k), generator=g, device=dev, dtype=torch.int32)
+    teacher = torch.empty(rows, k, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    out = ops.MusaTopKDistillationResult(torch.full((rows,), math.nan, device=dev),
+                                         torch.full_like(logits, math.nan))
+    ops.MusaTopKDistillation(logits, ids, teacher, out=out)
+    assert not bool(out.loss.isnan().any()) and not bool(out.backprop.isnan().any())
+    pick = some_rows(dev, rows, 1 << 26)
+    want = ops.MusaTopKDistillation(logits[pick], ids[pick], teacher[pick])
+    assert torch.equal(out.loss[pick], want.loss) and torch.equal(out.backprop[pick], want.backprop)
+
+
+def test_linear_copies_of_more_rows_than_a_grid_counts(dev):
+    """Ragged rows, copied to whole vectors first."""
+    m, k, n = (1 << 26) + 77, 9, 8
+    g = torch.Generator(device=dev).manual_seed(125)
+    x = torch.randint(-2, 3, (m, k), generator=g, device=dev, dtype=torch.int8).bfloat16()
+    w = torch.randint(-1, 2, (k, n), generator=g, device=dev).bfloat16()
+    y = ops.MusaLinear(x, w).y
+    assert torch.equal(y, (x.float() @ w.float()).bfloat16())  # whole numbers
+
+
+@pytest.mark.parametrize("tb", [False, True])
+def test_linear_of_one_row_and_the_most_columns(dev, tb):
+    """A product of few rows whose columns take more threads than a grid
+    counts, with either order of w."""
+    k, n = (3, (1 << 27) + 72) if tb else (1, (1 << 28) + 72)
+    g = torch.Generator(device=dev).manual_seed(126)
+    w = torch.randint(-1, 2, (n, k) if tb else (k, n), generator=g, device=dev, dtype=torch.int8).half()
+    x = torch.tensor([[2.0, -1.0, 3.0][:k]], device=dev).half()
+    out = ops.MusaLinearResult(torch.full((1, n), math.nan, dtype=torch.float16, device=dev), None)
+    ops.MusaLinear(x, w, transpose_b=tb, out=out)
+    assert ops.last_kernel_name() == "tfma_linear_few"
+    want = (w.float() * x[0].float()).sum(1) if tb else w[0].float() * 2
+    assert torch.equal(out.y[0], want.half())

@@ -424,7 +424,8 @@ int TFMA_MusaLinearGrad(void* stream, const TFMA_Tensor* y_backprop, const TFMA_
  * NULL): T [..., V], may replace logits.  An entry whose index is outside
  * [0, V) or whose logit is -inf is absent; a row without entries has loss 0
  * and gradient 0 whatever its logits.  An index that occurs twice counts with
- * both its entries.  A row of logits that are all -inf gives NaN.  K <= 1024. */
+ * both its entries.  A row of logits that are all -inf gives NaN.  K <= 1024.
+ * No workspace is needed: the query answers 0, and NULL and 0 will do. */
 int TFMA_MusaTopKDistillationWorkspaceBytes(const TFMA_Tensor* logits,
                                             const TFMA_Tensor* teacher_indices, size_t* bytes,
                                             TFMA_Status* status);

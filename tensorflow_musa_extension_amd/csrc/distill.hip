@@ -152,15 +152,15 @@ __device__ inline float soft(float x, float c, float top) {
   return __builtin_amdgcn_exp2f((x - top) * c);
 }
 
-// The gradient at the entries' places in [begin, end), over the q that the
-// workgroup has stored there: equal ids take the sum of their p, in order, at
-// the first of them.  `own` holds the entries' q.
+// The gradient at the entries' places, over the q that the workgroup has
+// stored there: equal ids take the sum of their p, in order, at the first of
+// them.  `own` holds the entries' q.
 template <class Tr, int kThreads>
 __device__ inline void place_entries(const DistillArgs& a, typename Tr::S* back, const Entries& e,
-                                     const float* own, float factor, int64_t begin, int64_t end) {
+                                     const float* own, float factor) {
   for (int j = threadIdx.x; j < a.k; j += kThreads) {
     const int32_t id = e.id[j];
-    if (id < begin || id >= end) continue;
+    if (id < 0) continue;
     float mass = 0.f;
     bool first = true;
     for (int i = 0; i < a.k; ++i) {
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
   });
   if (whole + tid < v) back[whole + tid] = Tr::st(scale * soft(rest, c2, top));
   __syncthreads();  // the stores above come before those below
-  place_entries<Tr, kThreads>(a, back, e, own, factor, 0, v);
+  place_entries<Tr, kThreads>(a, back, e, own, factor);
 }
 
 template <class Tr, int kThreads, int kPacks>
@@ -303,8 +303,6 @@ hipError_t by_width(const DistillArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
-
-size_t DistillWorkspaceBytes(DType t, int64_t rows, int64_t v) { return 0; }
 
 hipError_t LaunchDistill(DType t, const DistillArgs& a, hipStream_t stream) {
   if (a.rows == 0) return hipSuccess;

@@ -2053,7 +2053,7 @@ int TFMA_MusaTopKDistillationWorkspaceBytes(const TFMA_Tensor* logits,
   DistillArgs a{};
   if (const int rc = distill_geometry(logits, teacher_indices, &t, &a, status)) return rc;
   if (!bytes) return set_status(status, TFMA_INVALID_ARGUMENT, "bytes is null");
-  *bytes = DistillWorkspaceBytes(t, a.rows, a.v);
+  *bytes = 0;  // a row's state fits its workgroup
   return ok(status);
 }
 
@@ -2095,9 +2095,6 @@ int TFMA_MusaTopKDistillation(void* stream, const TFMA_Tensor* logits,
   if (const int rc = check_overlap(op, {{loss, "loss"}}, {{logits, "logits"}}, {}, status)) return rc;
   if (const int rc = check_overlap(op, {{backprop, "backprop"}}, {}, {{logits, "logits"}}, status))
     return rc;
-  if (const int rc = check_workspace(op, workspace, workspace_bytes,
-                                     DistillWorkspaceBytes(t, a.rows, a.v), status))
-    return rc;
   a.temperature = temperature;
   a.logits = logits->data;
   a.ids = teacher_indices->data;
@@ -2105,7 +2102,6 @@ int TFMA_MusaTopKDistillation(void* stream, const TFMA_Tensor* logits,
   a.weights = row_weights ? static_cast<const float*>(row_weights->data) : nullptr;
   a.loss = static_cast<float*>(loss->data);
   a.backprop = backprop ? backprop->data : nullptr;
-  a.workspace = workspace;
   return hip_status(status, LaunchDistill(t, a, as_stream(stream)), op);
 }
 

@@ -400,9 +400,7 @@ struct DistillArgs {
   const float* weights;  // may be null
   float* loss;
   void* backprop;  // may be null
-  void* workspace;
 };
-size_t DistillWorkspaceBytes(DType t, int64_t rows, int64_t v);
 hipError_t LaunchDistill(DType t, const DistillArgs& a, hipStream_t stream);
 
 }  // namespace tfma

@@ -616,8 +616,7 @@ def MusaTopKDistillation(logits, teacher_indices, teacher_logits, row_weights=No
             torch.empty_like(logits) if with_backprop else None)
     dl, di, dt = (_d(logits, "logits"), _d(teacher_indices, "teacher_indices"),
                   _d(teacher_logits, "teacher_logits"))
-    need = _query("TFMA_MusaTopKDistillationWorkspaceBytes", dl, di)
-    ws, ws_bytes, keep = _scratch(need, workspace, logits.device)
+    ws, ws_bytes, keep = _scratch(0, workspace, logits.device)  # none is needed
     _run("TFMA_MusaTopKDistillation", _cur(logits), dl, di, dt,
           _opt(row_weights, "row_weights"), float(temperature), _opt(out.loss, "loss"),
           _opt(out.backprop, "backprop"), ws, ws_bytes, keep=(keep,))

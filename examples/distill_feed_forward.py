@@ -97,9 +97,10 @@ class Block:
             self.half[n].copy_(v)
 
     def quantized(self):
-        """The weights for serving: e4m3 rows [outputs, inputs] and scales."""
+        """The weights that take a norm's 8-bit output, for serving: e4m3 rows
+        [outputs, inputs] and scales."""
         packed = {}
-        for name in ("up", "down", "embedding"):
+        for name in ("up", "embedding"):
             rows = self.matrices[name] if name == "embedding" else self.matrices[name].t()
             scale = rows.abs().amax(1) / 448
             packed[name] = ((rows / scale[:, None]).to(torch.float8_e4m3fn).contiguous(), scale)

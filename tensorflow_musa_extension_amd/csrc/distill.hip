@@ -177,10 +177,10 @@ __device__ inline void place_entries(const DistillArgs& a, typename Tr::S* back,
 // read again for each use.  The up to seven elements after the last whole pack
 // belong to the first threads, one each.
 // Bound by HBM where there are rows enough (4096 x 50304 bf16 with its gradient
-// 183 us, 4.5 TB/s of compulsory bytes; each workgroup reads, then computes
+// 184 us, 4.5 TB/s of compulsory bytes; each workgroup reads, then computes
 // two exponentials an element, then writes, so that reads and writes overlap
 // only between the rows that share a CU), else by one row's latency (61 x 50303
-// f32 without the gradient 8.4 us).
+// f32 without the gradient 8.3 us).
 template <class Tr, int kThreads, int kPacks>
 __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
   using S = typename Tr::S;
@@ -218,7 +218,10 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
       }
     } else {
 #pragma unroll 4
-      for (int c = tid * kPack; c < whole; c += kThreads * kPack) f(c, load_words<S>(x + c));
+      for (int c = tid * kPack; c < whole; c += kThreads * kPack) {
+        Words<S> w = load_words<S>(x + c);
+        f(c, w);
+      }
     }
   };
   float log_entries;
@@ -238,9 +241,17 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
   top = max_block<kThreads>(top, lds);
   const float c2 = per_temperature(kLog2E, a.temperature);
   float sum = soft(rest, c2, top);
-  each([&](int, const Words<S>& w) {
+  // Float rows in registers keep their exponentials in place of the logits, which
+  // the gradient then only scales (2000 x 50304 f32 182 us, 198 with them computed
+  // again).
+  constexpr bool kKeep = kPacks > 0 && sizeof(S) == 4;
+  each([&](int, Words<S>& w) {
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) sum += soft(element<Tr>(w, j), c2, top);
+    for (int j = 0; j < kPack; ++j) {
+      const float q = soft(element<Tr>(w, j), c2, top);
+      sum += q;
+      if constexpr (kKeep) w.w[j] = f32_bits(q);
+    }
   });
   sum = sum_block<kThreads>(sum, lds);
   const float weight = a.weights ? a.weights[row] : 1.f;
@@ -259,7 +270,10 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
     if (c >= whole) return;
     Pack<S> o;
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) o.v[j] = Tr::st(scale * soft(element<Tr>(w, j), c2, top));
+    for (int j = 0; j < kPack; ++j) {
+      const float q = element<Tr>(w, j);
+      o.v[j] = Tr::st(scale * (kKeep ? q : soft(q, c2, top)));
+    }
     *reinterpret_cast<Pack<S>*>(back + c) = o;
   });
   if (whole + tid < v) back[whole + tid] = Tr::st(scale * soft(rest, c2, top));

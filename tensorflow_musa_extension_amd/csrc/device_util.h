@@ -14,16 +14,20 @@ namespace tfma {
 // Grids of many workgroups.  A grid's threads along one dimension are counted
 // in 32 bits, and a launch of more wraps around without an error (2^24 + 5
 // workgroups of 256 threads run 5 of them).  many_groups lays `groups`
-// workgroups out in two dimensions; those past `groups` return at once.
+// workgroups out in as few equal rows as it takes; those past `groups`, fewer
+// than there are rows, return at once.  `across` is the grid's x, which the
+// kernel takes beside its other arguments: reading gridDim made 4 x 2048 norms
+// 3.9 us instead of 3.6.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kGroupsAcross = 1u << 20;  // of up to 1024 threads
-constexpr int64_t kMostGroups = int64_t(kGroupsAcross) * 65535;
+constexpr int64_t kGroupsAcross = 1 << 21;  // of up to 1024 threads
+constexpr int64_t kMostGroups = kGroupsAcross * 65535;
 inline dim3 many_groups(int64_t groups) {
-  if (groups <= kGroupsAcross) return dim3(static_cast<uint32_t>(groups));
-  return dim3(kGroupsAcross, static_cast<uint32_t>((groups + kGroupsAcross - 1) / kGroupsAcross));
+  const int64_t rows = (groups + kGroupsAcross - 1) / kGroupsAcross;
+  if (rows <= 1) return dim3(static_cast<uint32_t>(groups));
+  return dim3(static_cast<uint32_t>((groups + rows - 1) / rows), static_cast<uint32_t>(rows));
 }
-__device__ inline int64_t group_of_many() {
-  return int64_t(blockIdx.y) * kGroupsAcross + blockIdx.x;
+__device__ inline int64_t group_of_many(uint32_t across) {
+  return int64_t(blockIdx.y) * across + blockIdx.x;
 }
 
 // ---------------------------------------------------------------------------

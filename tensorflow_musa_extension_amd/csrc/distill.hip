@@ -189,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
   const Entries e = {reinterpret_cast<int32_t*>(dyn), dyn + a.k, dyn + 2 * a.k};
   float* own = dyn + 3 * a.k;
   const int tid = threadIdx.x;
-  const int64_t row = group_of_many();
+  const int64_t row = group_of_many(a.across);
   if (row >= a.rows) return;
   const S* x = static_cast<const S*>(a.logits) + row * a.v;
   const int v = static_cast<int>(a.v), whole = v & ~(kPack - 1);
@@ -282,10 +282,12 @@ __global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
 }
 
 template <class Tr, int kThreads, int kPacks>
-hipError_t launch(const DistillArgs& a, hipStream_t stream) {
+hipError_t launch(DistillArgs a, hipStream_t stream) {
   if (a.rows > kMostGroups) return hipErrorInvalidConfiguration;
-  TFMA_LAUNCH("tfma_distill", (distill_kernel<Tr, kThreads, kPacks>), many_groups(a.rows),
-              dim3(kThreads), 4 * a.k * sizeof(float), stream, a);
+  const dim3 grid = many_groups(a.rows);
+  a.across = grid.x;
+  TFMA_LAUNCH("tfma_distill", (distill_kernel<Tr, kThreads, kPacks>), grid, dim3(kThreads),
+              4 * a.k * sizeof(float), stream, a);
   return hipGetLastError();
 }
 

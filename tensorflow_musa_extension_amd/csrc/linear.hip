@@ -636,7 +636,8 @@ struct Config {
   static constexpr bool kTurned = kTurned_;
   // A tile's longest rows end below DirectTile::kOutside, which no sum of an
   // offset and the way down from it then passes by 2^32 either.
-  static_assert((kTM_ > kTN_ ? kTM_ : kTN_) * kLinear8MaxK <= int64_t(1) << 31, "offsets in 31 bits");
+  static_assert((kTM_ > kTN_ ? kTM_ : kTN_) * kLinear8MaxK <= int64_t(1) << 31,
+                "offsets in 31 bits");
   static constexpr int kTM = kTM_, kTN = kTN_, kWavesM = kWavesM_, kWavesN = kWavesN_,
                        kSlots = kSlots_, kWaves = kWavesM * kWavesN;
   static constexpr int kFM = kTM / kWavesM / 16, kFN = kTN / kWavesN / 16;  // fragments of a wave
@@ -811,10 +812,11 @@ __global__ __launch_bounds__(Cf::kWaves * 64) void direct_kernel(GemmShape s, It
 // Adds the splits' sums, which are float, in order and finishes them.  About 3 us
 // for little data.
 template <class Tr>
-__global__ __launch_bounds__(256) void join_kernel(int64_t m, int64_t n, int splits,
-                                                   const float* partial, LinearEpilogue e) {
+__global__ __launch_bounds__(256) void join_kernel(uint32_t across, int64_t m, int64_t n,
+                                                   int splits, const float* partial,
+                                                   LinearEpilogue e) {
   const int64_t per_row = (n + 7) / 8;
-  const int64_t i = group_of_many() * 256 + threadIdx.x;
+  const int64_t i = group_of_many(across) * 256 + threadIdx.x;
   if (i >= m * per_row) return;
   const int64_t row = i / per_row, col = i % per_row * 8;
   const float* p = partial + row * n + col;
@@ -840,8 +842,9 @@ template <class Tr>
 hipError_t launch_join(const GemmShape& s, int splits, const void* workspace, const LinearEpilogue& e,
                        hipStream_t stream) {
   const int64_t groups = (s.m * ((s.n + 7) / 8) + 255) / 256;
-  TFMA_LAUNCH("tfma_linear_join", join_kernel<Tr>, many_groups(groups), dim3(256), 0, stream, s.m,
-              s.n, splits, static_cast<const float*>(workspace), e);
+  const dim3 grid = many_groups(groups);
+  TFMA_LAUNCH("tfma_linear_join", join_kernel<Tr>, grid, dim3(256), 0, stream, grid.x, s.m, s.n,
+              splits, static_cast<const float*>(workspace), e);
   return hipGetLastError();
 }
 
@@ -907,9 +910,9 @@ __device__ inline void load_row(const S* __restrict__ p, int64_t ld, int64_t row
 }
 
 template <class Op, class Tr, bool kBKC, int kMT, int kNJ, int kWaves>
-__global__ __launch_bounds__(kWaves * 64) void few_rows_kernel(GemmShape s, int splits, int steps,
-                                                              const void* a_, const void* b_,
-                                                              LinearEpilogue ep, float* partial) {
+__global__ __launch_bounds__(kWaves * 64) void few_rows_kernel(
+    GemmShape s, uint32_t across, int splits, int steps, const void* a_, const void* b_,
+    LinearEpilogue ep, float* partial) {
   using S = typename Op::S;
   using Frag = typename Op::Frag;
   constexpr int kE = sizeof(S), kChunk = 16 / kE, kCols = 16 * kNJ;
@@ -922,7 +925,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_rows_kernel(GemmShape s, int 
   const S* a = static_cast<const S*>(a_);
   const S* b = static_cast<const S*>(b_);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const uint32_t group = static_cast<uint32_t>(group_of_many());
+  const uint32_t group = static_cast<uint32_t>(group_of_many(across));
   const int tile = group / splits, split = group % splits;
   const int64_t n0 = int64_t(tile) * kCols;
   if (n0 >= s.n) return;
@@ -1088,10 +1091,10 @@ hipError_t launch_few(const GemmShape& s, const void* a, const void* b, const Li
   constexpr bool kWide = sizeof(typename Op::S) > 1;  // e4m3 operands never need 32 rows
   if (!kWide || s.m <= 16)
     TFMA_LAUNCH("tfma_linear_few", (few_rows_kernel<Op, Tr, kBKC, 1, kNJ, kFewWaves>), grid, block, 0,
-                stream, s, splits, steps, a, b, e, partial);
+                stream, s, grid.x, splits, steps, a, b, e, partial);
   else if constexpr (kWide)
     TFMA_LAUNCH("tfma_linear_few", (few_rows_kernel<Op, Tr, kBKC, 2, kNJ, kFewWaves>), grid, block, 0,
-                stream, s, splits, steps, a, b, e, partial);
+                stream, s, grid.x, splits, steps, a, b, e, partial);
   if (const hipError_t err = hipGetLastError(); err != hipSuccess || splits == 1) return err;
   return launch_join<Tr>(s, splits, workspace, e, stream);
 }
@@ -1159,6 +1162,7 @@ struct PadArgs {
   void* to[2];
   int64_t rows[2], cols[2], ld[2];
   uint32_t groups0, groups;  // workgroups of the first operand, and of both
+  uint32_t across;  // the launch's, of many_groups
 };
 __host__ __device__ inline uint32_t pad_pieces(int64_t ld, int esize) {
   return static_cast<uint32_t>((ld * esize + 1023) / 1024);
@@ -1166,7 +1170,7 @@ __host__ __device__ inline uint32_t pad_pieces(int64_t ld, int esize) {
 template <typename S>
 __global__ __launch_bounds__(256) void pad_kernel(PadArgs p) {
   constexpr int kN = 16 / static_cast<int>(sizeof(S));
-  const uint32_t group = static_cast<uint32_t>(group_of_many());
+  const uint32_t group = static_cast<uint32_t>(group_of_many(p.across));
   if (group >= p.groups) return;
   const int which = group < p.groups0 ? 0 : 1;
   const uint32_t piece = (group - (which ? p.groups0 : 0)) * 4 + (threadIdx.x >> 6);
@@ -1232,7 +1236,9 @@ hipError_t launch_pad(const GemmShape& s, const Padding& p, const void*& a, cons
   if (groups >= (int64_t(1) << 30)) return hipErrorInvalidConfiguration;
   args.groups0 = static_cast<uint32_t>(groups0);
   args.groups = static_cast<uint32_t>(groups);
-  TFMA_LAUNCH("tfma_linear_pad", pad_kernel<S>, many_groups(groups), dim3(256), 0, stream, args);
+  const dim3 grid = many_groups(groups);
+  args.across = grid.x;
+  TFMA_LAUNCH("tfma_linear_pad", pad_kernel<S>, grid, dim3(256), 0, stream, args);
   return hipGetLastError();
 }
 

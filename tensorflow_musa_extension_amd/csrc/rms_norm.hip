@@ -119,7 +119,7 @@ template <class Tr, int kThreads, int kPacks>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void norm_kernel(RmsNormArgs a) {
   __shared__ float lds[kThreads / 64];
   constexpr int kRows = kThreads < 256 ? 256 / kThreads : 1;
-  const int64_t row = group_of_many() * kRows + threadIdx.x / kThreads;
+  const int64_t row = group_of_many(a.across) * kRows + threadIdx.x / kThreads;
   if (row >= a.rows) return;  // whole waves, and whole workgroups of one row
   const int tid = threadIdx.x % kThreads;
   const int n = static_cast<int>(a.c);
@@ -187,7 +187,7 @@ template <class Tr>
 __global__ __launch_bounds__(1024) void norm_long_kernel(RmsNormArgs a) {
   constexpr int kThreads = 1024;
   __shared__ float lds[kThreads / 64];
-  const int64_t row = group_of_many();
+  const int64_t row = group_of_many(a.across);
   if (row >= a.rows) return;
   const int64_t at = row * a.c;
   const int n = static_cast<int>(a.c);
@@ -249,12 +249,14 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(RmsNormArgs a) {
 }
 
 template <class Tr, int kThreads, int kPacks>
-hipError_t launch_norm(const RmsNormArgs& a, hipStream_t stream) {
+hipError_t launch_norm(RmsNormArgs a, hipStream_t stream) {
   constexpr int kRows = kThreads < 256 ? 256 / kThreads : 1;
   const int64_t groups = (a.rows + kRows - 1) / kRows;
   if (groups > kMostGroups) return hipErrorInvalidConfiguration;
-  TFMA_LAUNCH("tfma_rms_norm", (norm_kernel<Tr, kThreads, kPacks>), many_groups(groups),
-              dim3(kRows * kThreads), 0, stream, a);
+  const dim3 grid = many_groups(groups);
+  a.across = grid.x;
+  TFMA_LAUNCH("tfma_rms_norm", (norm_kernel<Tr, kThreads, kPacks>), grid, dim3(kRows * kThreads), 0,
+              stream, a);
   return hipGetLastError();
 }
 
@@ -263,7 +265,7 @@ hipError_t launch_norm(const RmsNormArgs& a, hipStream_t stream) {
 // 8192 48.7 against 53.4 for 256 threads of four).  Rows of up to 1024 take one
 // wave and no barrier (30000 x 1000 bf16 48.8 us against 63.2 for 256 threads).
 template <class Tr>
-hipError_t norm_by_width(const RmsNormArgs& a, hipStream_t stream) {
+hipError_t norm_by_width(RmsNormArgs a, hipStream_t stream) {
   if (a.c <= 64 * 8) return launch_norm<Tr, 64, 1>(a, stream);
   if (a.c <= 64 * 16) return launch_norm<Tr, 64, 2>(a, stream);
   if (a.c <= 256 * 8) return launch_norm<Tr, 256, 1>(a, stream);
@@ -271,8 +273,9 @@ hipError_t norm_by_width(const RmsNormArgs& a, hipStream_t stream) {
   if (a.c <= 1024 * 8) return launch_norm<Tr, 1024, 1>(a, stream);
   if (a.c <= 1024 * 16) return launch_norm<Tr, 1024, 2>(a, stream);
   if (a.rows > kMostGroups) return hipErrorInvalidConfiguration;
-  TFMA_LAUNCH("tfma_rms_norm_long", norm_long_kernel<Tr>, many_groups(a.rows), dim3(1024), 0, stream,
-              a);
+  const dim3 grid = many_groups(a.rows);
+  a.across = grid.x;
+  TFMA_LAUNCH("tfma_rms_norm_long", norm_long_kernel<Tr>, grid, dim3(1024), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -420,11 +423,11 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(RmsNormGradArgs a,
 
 // Sums `partial` over its groups: a workgroup has 64 columns, its sixteen
 // waves take groups in turn.
-__global__ __launch_bounds__(1024) void gamma_sums_kernel(int64_t groups, int64_t c,
+__global__ __launch_bounds__(1024) void gamma_sums_kernel(uint32_t across, int64_t groups, int64_t c,
                                                           const float* partial, float* out) {
   __shared__ float sums[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t i = group_of_many() * 64 + lane;
+  const int64_t i = group_of_many(across) * 64 + lane;
   float s = 0.f;
   if (i < c) {
 #pragma unroll 8
@@ -487,8 +490,9 @@ hipError_t norm_grad(const RmsNormGradArgs& a, hipStream_t stream) {
     const hipError_t e = norm_grad_by_width<Tr>(b, groups, rows_per, stream);
     if (e != hipSuccess || groups == 1) return e;
   }
-  TFMA_LAUNCH("tfma_rms_norm_dgamma", gamma_sums_kernel, many_groups((a.c + 63) / 64), dim3(1024), 0,
-              stream, groups, a.c, a.partial, a.dgamma);
+  const dim3 grid = many_groups((a.c + 63) / 64);
+  TFMA_LAUNCH("tfma_rms_norm_dgamma", gamma_sums_kernel, grid, dim3(1024), 0, stream, grid.x, groups,
+              a.c, a.partial, a.dgamma);
   return hipGetLastError();
 }
 

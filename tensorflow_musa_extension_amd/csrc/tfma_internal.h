@@ -363,6 +363,7 @@ hipError_t LaunchLinearDz(DType t, int64_t m, int64_t n, int act, const void* dy
 struct RmsNormArgs {
   int64_t rows, c;
   float epsilon;
+  uint32_t across;  // the launch's, of many_groups
   const void* x;
   const void* residual;  // may be null
   const float* gamma;
@@ -391,6 +392,7 @@ constexpr int kDistillMaxK = 1024;  // teacher entries of one row
 struct DistillArgs {
   int64_t rows, v;
   int k;
+  uint32_t across;  // the launch's, of many_groups
   bool ids64;
   bool teacher_f32;  // else the logits' type
   float temperature;
